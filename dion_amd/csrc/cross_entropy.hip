@@ -15,11 +15,15 @@ namespace {
 
 constexpr float QUIET_NAN = __builtin_nanf("");
 constexpr float LOG2E = 1.44269504088896340736f;
+// How a kernel takes the logits' cap.
+enum Cap : int {
+  NONE,    // z = x
+  SMALL,   // bf16 logits and at most SMALL_CAP: z by a reciprocal alone, and no maximum
+  WIDE,    // any other cap: z as exact as x
+};
 // Up to this cap no maximum is looked for in bf16 logits: they lie between -cap and cap, and the sum of exp(z - cap), at least
-// exp(-80), serves like that of exp(z - maximum).  (Of fp32 logits it would cost the last bits of the large terms.)
+// exp(-80), serves like that of exp(z - maximum).
 constexpr float SMALL_CAP = 40.f;
-template <typename T, bool CAP>
-__device__ __forceinline__ bool needs_max(float cap) { return !CAP || sizeof(T) == 4 || cap > SMALL_CAP; }
 constexpr float NO_MAX = -__builtin_inff();
 constexpr int COUNT_BLOCKS = 64;   // partial counts of the rows that count: one a lane where they are added up
 constexpr int SLICES = 64;         // slices of a row at most: one a lane where their sums are joined
@@ -51,25 +55,27 @@ struct CeArgs {
 
 __device__ __forceinline__ float fast_exp(float d) { return __builtin_amdgcn_exp2f(d * LOG2E); }
 
-// exp(z - ref) for z = cap tanh(x / cap), or z = x, and the derivative dz/dx.
+// z = cap tanh(x / cap), or z = x, and the derivative dz/dx.
 //
-// With r = 1 / (1 + exp(2 u)), u = x / cap: tanh u = 1 - 2 r and 1 - tanh^2 u = 4 r (1 - r).  That is within a few 2^-24 of the
-// hyperbolic tangent in absolute terms, which the softmax of bf16 logits does not show, and exp(z - ref) is then one multiply-add and
-// one exponential of r.  fp32 logits take the series of the tangent up to u^11 where |u| < 0.3, so that small ones keep their last
-// bits, and subtract before they scale.
-template <typename T, bool CAP>
+// With r = 1 / (1 + exp(2 u)), u = x / cap: tanh u = 1 - 2 r and 1 - tanh^2 u = 4 r (1 - r).  That z is off by up to some 2^-22 of the
+// cap, however small it is itself, since the terms are of the cap's size.  A SMALL cap leaves it at that, 1e-5 at the most, and
+// exp(z - ref) is then one multiply-add and one exponential of r: of 2048 rows of bf16 logits of deviation 2 the losses are 8.8e-7,
+// 1.7e-6 and 2.4e-6 off in the root mean square with caps of 15, 30 and 40, and 4.5e-7 if they are taken as WIDE, which costs half as much
+// again where the arithmetic bounds a kernel (8192 rows of 50304 classes with the gradient 380 and 560 us).  WIDE caps and fp32
+// logits take the series of the tangent up to u^11 where |u| < 0.3, off by a few 2^-24 of z itself whatever the cap, and subtract before
+// they scale.
+template <Cap CAP>
 struct Capped {
-  float r = 0.f, z = 0.f, slope = 1.f;   // of bf16 r alone, unless z or the slope is asked for
-  static constexpr bool EXACT = sizeof(T) == 4;
+  float r = 0.f, z = 0.f, slope = 1.f;   // of a SMALL cap r alone, unless z or the slope is asked for
   __device__ __forceinline__ Capped(const CeArgs& a, float x) {
-    if (!CAP) {
+    if (CAP == NONE) {
       z = x;
       return;
     }
     r = __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(x * a.exp_scale));
     z = fmaf(-2.f * a.cap, r, a.cap);
     slope = 4.f * fmaf(-r, r, r);
-    if (EXACT) {
+    if (CAP == WIDE) {
       const float u = x * a.inv_cap, q = u * u;
       float p = fmaf(q, -1382.f / 155925.f, 62.f / 2835.f);
       p = fmaf(q, p, -17.f / 315.f);
@@ -83,16 +89,16 @@ struct Capped {
     }
   }
 };
-template <typename T, bool CAP>
-__device__ __forceinline__ float capped(const CeArgs& a, float x) { return Capped<T, CAP>(a, x).z; }
+template <Cap CAP>
+__device__ __forceinline__ float capped(const CeArgs& a, float x) { return Capped<CAP>(a, x).z; }
 
 // exp(z - ref), ref fixed for a row.
-template <typename T, bool CAP>
+template <Cap CAP>
 struct Exponential {
   float ref, shift, scale;
   __device__ __forceinline__ Exponential(const CeArgs& a, float ref) : ref(ref), shift((a.cap - ref) * LOG2E), scale(-2.f * LOG2E * a.cap) {}
-  __device__ __forceinline__ float operator()(const Capped<T, CAP>& c) const {
-    if (CAP && !Capped<T, CAP>::EXACT) return __builtin_amdgcn_exp2f(fmaf(scale, c.r, shift));
+  __device__ __forceinline__ float operator()(const Capped<CAP>& c) const {
+    if (CAP == SMALL) return __builtin_amdgcn_exp2f(fmaf(scale, c.r, shift));
     return fast_exp(c.z - ref);
   }
 };
@@ -167,14 +173,14 @@ __device__ __forceinline__ Weights weights(const CeArgs& a, long long row, float
 }
 
 // Gradient of N classes from `first` on, in place of their logits.
-template <typename T, bool CAP, int N>
-__device__ __forceinline__ void gradient(const CeArgs& a, float (&x)[N], int first, long long target, const Exponential<T, CAP>& e, Weights g) {
+template <Cap CAP, int N>
+__device__ __forceinline__ void gradient(const CeArgs& a, float (&x)[N], int first, long long target, const Exponential<CAP>& e, Weights g) {
 #pragma unroll
   for (int i = 0; i < N; ++i) {
-    const Capped<T, CAP> c(a, x[i]);
+    const Capped<CAP> c(a, x[i]);
     float d = g.wp * e(c);
     if ((unsigned long long)(target - first) < N && first + i == target) d -= g.w;
-    x[i] = CAP ? d * c.slope : d;
+    x[i] = CAP == NONE ? d : d * c.slope;
   }
 }
 
@@ -187,7 +193,7 @@ __device__ __forceinline__ void gradient(const CeArgs& a, float (&x)[N], int fir
 // two passes).  19 cycles a lane and element without a cap, 36 with one in bf16, where the arithmetic bounds it (4.4 TB/s).  Two
 // workgroups a compute unit take turns at memory and arithmetic; rows of more than 8192 vectors leave room for one (4.0 TB/s with 18992
 // vectors: 2048 rows of 151936 bf16 classes in 312 us, 383 if they are read twice).
-template <typename T, bool CAP, int THREADS, int VECS>
+template <typename T, Cap CAP, int THREADS, int VECS>
 __global__ __launch_bounds__(THREADS) void ce_row_kernel(CeArgs a) {
   constexpr int N = 16 / sizeof(T);
   const long long row = blockIdx.x;
@@ -220,7 +226,7 @@ __global__ __launch_bounds__(THREADS) void ce_row_kernel(CeArgs a) {
   const float share = count_share(a, THREADS);
 
   float m = a.cap;
-  if (needs_max<T, CAP>(a.cap)) {
+  if (CAP != SMALL) {
     m = last;
     if (vecs) {
 #pragma unroll
@@ -231,9 +237,9 @@ __global__ __launch_bounds__(THREADS) void ce_row_kernel(CeArgs a) {
         for (int i = 0; i < N; ++i) m = fmaxf(m, z[i]);
       }
     }
-    m = capped<T, CAP>(a, m);   // (it rises with its argument)
+    m = capped<CAP>(a, m);   // (it rises with its argument)
   }
-  const Exponential<T, CAP> from_max(a, reference(m));
+  const Exponential<CAP> from_max(a, reference(m));
   float s = ends ? from_max({a, last}) : 0.f;
 #pragma unroll
   for (int j = 0; j < VECS; ++j) {
@@ -249,25 +255,25 @@ __global__ __launch_bounds__(THREADS) void ce_row_kernel(CeArgs a) {
   if (a.counts) count = da_group_sum(share);
   const float lse = m + logf(s);
   if (threadIdx.x == 0) {
-    a.losses[row] = row_loss(a, lse, capped<T, CAP>(a, xt), known);
+    a.losses[row] = row_loss(a, lse, capped<CAP>(a, xt), known);
     if (a.lse) a.lse[row] = lse;
   }
   if (!a.dx) return;
   const Weights g = weights(a, row, lse, known, count);
-  const Exponential<T, CAP> from_lse(a, lse);
+  const Exponential<CAP> from_lse(a, lse);
 #pragma unroll
   for (int j = 0; j < VECS; ++j) {
     const int v = j * THREADS + (int)threadIdx.x;
     if (v < vecs) {
       float z[N];
       raw[j].get(z);
-      gradient<T, CAP>(a, z, v * N, target, from_lse, g);
+      gradient<CAP>(a, z, v * N, target, from_lse, g);
       da_store(dx + v * N, 0, z);
     }
   }
   if (ends) {
     float z[1] = {last};
-    gradient<T, CAP>(a, z, end, target, from_lse, g);
+    gradient<CAP>(a, z, end, target, from_lse, g);
     st_from_float(dx + end, z[0]);
   }
 }
@@ -280,7 +286,7 @@ __global__ __launch_bounds__(THREADS) void ce_row_kernel(CeArgs a) {
 constexpr int SLICE_THREADS = 1024, SLICE_VECS = 4;
 
 // Maximum and sum of one slice of a row; of a row in one slice also its loss.
-template <typename T, bool CAP>
+template <typename T, Cap CAP>
 __global__ __launch_bounds__(SLICE_THREADS) void ce_slice_kernel(CeArgs a) {
   constexpr int N = 16 / sizeof(T);
   const long long row = blockIdx.x / a.slices;
@@ -296,7 +302,7 @@ __global__ __launch_bounds__(SLICE_THREADS) void ce_slice_kernel(CeArgs a) {
   const T* x = static_cast<const T*>(a.x) + row * a.ld;
   const int begin = slice * a.slice, end = slice + 1 < a.slices ? begin + a.slice : a.vocab;
   const int vecs = (end - begin) / N;
-  float top = NO_MAX, m = needs_max<T, CAP>(a.cap) ? capped<T, CAP>(a, top) : a.cap, s = 0.f;   // top: before the cap
+  float top = NO_MAX, m = CAP == SMALL ? a.cap : capped<CAP>(a, top), s = 0.f;   // top: before the cap
   constexpr int STEP = SLICE_THREADS * SLICE_VECS;
   DaVec<T, N> next[SLICE_VECS];
   auto request = [&](int base) {
@@ -315,16 +321,16 @@ __global__ __launch_bounds__(SLICE_THREADS) void ce_slice_kernel(CeArgs a) {
     float z[SLICE_VECS][N];
 #pragma unroll
     for (int j = 0; j < SLICE_VECS; ++j) here[j].get(z[j]);
-    if (needs_max<T, CAP>(a.cap)) {
+    if (CAP != SMALL) {
 #pragma unroll
       for (int j = 0; j < SLICE_VECS; ++j)
 #pragma unroll
         for (int i = 0; i < N; ++i) top = fmaxf(top, z[j][i]);   // (a repeated vector changes no maximum)
-      const float nm = capped<T, CAP>(a, top);
+      const float nm = capped<CAP>(a, top);
       s *= fast_exp(m - reference(nm));
       m = nm;
     }
-    const Exponential<T, CAP> from_max(a, reference(m));
+    const Exponential<CAP> from_max(a, reference(m));
 #pragma unroll
     for (int j = 0; j < SLICE_VECS; ++j) {
       if (base + j * SLICE_THREADS + (int)threadIdx.x < vecs) {
@@ -334,7 +340,7 @@ __global__ __launch_bounds__(SLICE_THREADS) void ce_slice_kernel(CeArgs a) {
     }
   }
   if (vecs * N + (int)threadIdx.x < end - begin) {
-    const float z = capped<T, CAP>(a, ld_as_float(x + begin + vecs * N + threadIdx.x)), nm = fmaxf(m, z);
+    const float z = capped<CAP>(a, ld_as_float(x + begin + vecs * N + threadIdx.x)), nm = fmaxf(m, z);
     s = s * fast_exp(m - reference(nm)) + fast_exp(z - reference(nm));
     m = nm;
   }
@@ -342,7 +348,7 @@ __global__ __launch_bounds__(SLICE_THREADS) void ce_slice_kernel(CeArgs a) {
   block_join<SLICE_THREADS>(m, s, none);
   if (threadIdx.x) return;
   const bool known = target >= 0 && target < a.vocab;
-  const float zt = capped<T, CAP>(a, ld_as_float(x + (known ? target : 0)));
+  const float zt = capped<CAP>(a, ld_as_float(x + (known ? target : 0)));
   if (a.slices > 1) {
     a.partial[row * a.slices + slice] = make_float2(m, s);
     if (slice == 0) a.target_logit[row] = zt;
@@ -384,7 +390,7 @@ constexpr int GRAD_THREADS = 256, GRAD_VECS = 4;
 // way at once, and a compute unit four workgroups at different points of their work: 8192 rows of 50304 bf16 classes 286 us (5.8 TB/s),
 // with a cap 296; in slices of twice as many vectors, half of them at a time, 303 and 332, half of them ahead 314 and 319, all of
 // them at once 306 and 309; 512 threads 295 and 292.
-template <typename T, bool CAP>
+template <typename T, Cap CAP>
 __global__ __launch_bounds__(GRAD_THREADS) void ce_grad_kernel(CeArgs a) {
   constexpr int N = 16 / sizeof(T);
   const long long row = blockIdx.x / a.slices;
@@ -414,18 +420,18 @@ __global__ __launch_bounds__(GRAD_THREADS) void ce_grad_kernel(CeArgs a) {
       if (a.lse) a.lse[row] = lse;
     }
   }
-  const Exponential<T, CAP> from_lse(a, lse);
+  const Exponential<CAP> from_lse(a, lse);
 #pragma unroll
   for (int j = 0; j < GRAD_VECS; ++j) {
     const int v = j * GRAD_THREADS + (int)threadIdx.x;
     if (v >= vecs) break;
     float z[N];
     raw[j].get(z);
-    if (!ignored) gradient<T, CAP>(a, z, begin + v * N, target, from_lse, g);
+    if (!ignored) gradient<CAP>(a, z, begin + v * N, target, from_lse, g);
     da_store(dx + v * N, 0, z);
   }
   if (ends) {
-    if (!ignored) gradient<T, CAP>(a, last, begin + tail, target, from_lse, g);
+    if (!ignored) gradient<CAP>(a, last, begin + tail, target, from_lse, g);
     st_from_float(dx + tail, last[0]);
   }
 }
@@ -526,7 +532,7 @@ Plan plan(long long rows, long long vocab, int dtype) {
 int check_args(const void* logits, int dtype, long long ld, const void* targets, int index_bits, long long rows, long long vocab,
                float softcap, int reduction) {
   if (rows < 0 || vocab <= 0 || ld < vocab || (index_bits != 32 && index_bits != 64)) return DA_ERR_ARG;
-  if (softcap != 0.f && !(softcap > 1e-30f && softcap < 1e30f)) return DA_ERR_ARG;   // (its reciprocal is needed)
+  if (softcap != 0.f && !(softcap >= 1e-30f && softcap <= 1e30f)) return DA_ERR_ARG;   // (its reciprocal is needed)
   if (reduction != DION_AMD_REDUCE_NONE && reduction != DION_AMD_REDUCE_SUM && reduction != DION_AMD_REDUCE_MEAN) return DA_ERR_ARG;
   if (!da_float_dtype(dtype)) return DA_ERR_DTYPE;
   if (rows >= MAX_ROWS || vocab > MAX_VOCAB) return DA_ERR_LIMIT;
@@ -546,10 +552,11 @@ void launch_count(CeArgs& a, float* counts, hipStream_t s) {
 
 #define DA_CE(LAUNCH)                                                                                                        \
   do {                                                                                                                       \
-    if (dtype == DA_BF16 && a.cap > 0.f) LAUNCH(bf16_t, true);                                                               \
-    else if (dtype == DA_BF16) LAUNCH(bf16_t, false);                                                                        \
-    else if (a.cap > 0.f) LAUNCH(float, true);                                                                               \
-    else LAUNCH(float, false);                                                                                               \
+    if (dtype == DA_BF16 && a.cap > SMALL_CAP) LAUNCH(bf16_t, WIDE);                                                         \
+    else if (dtype == DA_BF16 && a.cap > 0.f) LAUNCH(bf16_t, SMALL);                                                         \
+    else if (dtype == DA_BF16) LAUNCH(bf16_t, NONE);                                                                         \
+    else if (a.cap > 0.f) LAUNCH(float, WIDE);                                                                               \
+    else LAUNCH(float, NONE);                                                                                                \
   } while (0)
 #define DA_CE_SLICES(kernel, threads) hipLaunchKernelGGL(kernel, dim3((unsigned)(a.rows * a.slices)), dim3(threads), 0, s, a)
 #define DA_CE_STATS(T, CAP) DA_CE_SLICES((ce_slice_kernel<T, CAP>), SLICE_THREADS)

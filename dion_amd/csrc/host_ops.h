@@ -300,7 +300,7 @@ struct LossCall {
     rows = targets.numel();
     x = rows_of(logits.reshape({rows, vocab}));
     t = targets.contiguous();
-    if (o.cap != 0.f && !(o.cap > 1e-30f && o.cap < 1e30f)) refuse(op, "softcap must be zero or a positive number between 1e-30 and 1e30");
+    if (o.cap != 0.f && !(o.cap >= 1e-30f && o.cap <= 1e30f)) refuse(op, "softcap must be zero or a positive number between 1e-30 and 1e30");
   }
 };
 

@@ -1,0 +1,46 @@
+"""The operators of the model over ranges that ordinary sizes and values do not reach: large soft caps, long rows and lists, what
+autograd has to be told, limits of the index arithmetic.
+
+Bounds are those of the arithmetic, as in test_gpu_model_ops."""
+import math
+
+import pytest
+import torch
+
+from test_gpu_model_ops import BF, EPS, F32, _gen, _loss_problem, _qk_problem, _within
+
+pytestmark = pytest.mark.gpu
+
+
+# -------------------------------------------------------------------------------------------------------- cross entropy
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("rows, vocab", [(40, 1000), (70, 70001), (2, 131072)])
+@pytest.mark.parametrize("softcap", [50.0, 1e4, 1e6, 1e20, 1e30])
+def test_cross_entropy_with_large_caps(dev, dtype, rows, vocab, softcap):
+    """A capped logit is off by rounded operations on itself, whatever the cap: x / cap by two products with rounded factors (3), its
+    exponential and what follows from it at most 21 units of 2^-24 of the logit where |x| >= 0.3 cap, below that a polynomial (6)."""
+    from dion_amd import cross_entropy, cross_entropy_with_grad
+    from oracle import model_ops as O
+
+    logits, targets = _loss_problem(rows, vocab, dtype, seed=rows)
+    targets[0] = 0
+    x, t = logits.to(dev), targets.to(dev)
+    live = targets != -100
+    losses, lse = O.cross_entropy(logits, targets, softcap=softcap)
+    z = O.capped(logits.double(), softcap)
+    off = 24 * EPS * logits.double().abs().clamp(max=softcap)
+    dlse = (vocab / 64 + 44) * 2 * EPS + 2 * EPS * lse.abs() + off.max(-1).values
+    at = targets.clamp(min=0)[:, None]
+    slack = torch.where(live, dlse + off.gather(-1, at)[:, 0] + 2 * EPS * z.gather(-1, at)[:, 0].abs(), 0.0)
+    far = (z - lse[:, None]).abs().clamp(max=200)
+    dslack = torch.exp(z - lse[:, None]) * (dlse[:, None] + off + (2 * far + 28) * EPS)
+    dslack.scatter_add_(-1, at, torch.full_like(lse, 24 * EPS)[:, None])
+
+    _within(cross_entropy(x, t, reduction="none", softcap=softcap), losses, slack, "losses")
+    want = O.cross_entropy_grad(logits, targets, 1.0, softcap=softcap)
+    loss, dx = cross_entropy_with_grad(x, t, reduction="sum", softcap=softcap)
+    _within(loss, losses.sum(), slack.sum(), "sum")
+    _within(dx, want, dslack + 4 * EPS * want.abs(), "gradient")
+    leaf = x.clone().requires_grad_(True)
+    cross_entropy(leaf, t, reduction="sum", softcap=softcap).backward()
+    _within(leaf.grad, want, dslack + 4 * EPS * want.abs(), "autograd")
