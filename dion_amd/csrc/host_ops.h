@@ -280,7 +280,8 @@ void run_qk_norm_rope_grad(const QkInputs& in, const at::Tensor (&dy)[2], at::Te
 
 struct LossOptions {
   long long ignore;
-  float cap, z_loss;
+  double cap;   // as the caller gave it: what float32 rounds to zero would be no cap
+  float z_loss;
   int reduction;
 };
 
@@ -300,7 +301,7 @@ struct LossCall {
     rows = targets.numel();
     x = rows_of(logits.reshape({rows, vocab}));
     t = targets.contiguous();
-    if (o.cap != 0.f && !(o.cap >= 1e-30f && o.cap <= 1e30f)) refuse(op, "softcap must be zero or a positive number between 1e-30 and 1e30");
+    if (o.cap != 0.0 && !(o.cap >= 1e-30 && o.cap <= 1e30)) refuse(op, "softcap must be zero or a positive number between 1e-30 and 1e30");
   }
 };
 
@@ -325,7 +326,7 @@ void run_cross_entropy(const at::Tensor& logits, const at::Tensor& targets, cons
   int rc;
   {
     const Released released;
-    rc = ops.cross_entropy(c.x.data_ptr(), c.code, pitch(c.x), c.t.data_ptr(), c.bits, c.rows, c.vocab, o.ignore, o.cap, o.z_loss,
+    rc = ops.cross_entropy(c.x.data_ptr(), c.code, pitch(c.x), c.t.data_ptr(), c.bits, c.rows, c.vocab, o.ignore, (float)o.cap, o.z_loss,
                            o.reduction, out[0].data_ptr<float>(), keep ? out[1].data_ptr<float>() : nullptr,
                            gradient ? out[2].data_ptr() : nullptr, ldd, scale, ws.get(), need, stream_of(c.x.device()));
   }
@@ -342,7 +343,7 @@ at::Tensor run_cross_entropy_grad(const at::Tensor& logits, const at::Tensor& ta
   int rc;
   {
     const Released released;
-    rc = ops.cross_entropy_grad(c.x.data_ptr(), c.code, pitch(c.x), c.t.data_ptr(), c.bits, c.rows, c.vocab, o.ignore, o.cap, o.z_loss,
+    rc = ops.cross_entropy_grad(c.x.data_ptr(), c.code, pitch(c.x), c.t.data_ptr(), c.bits, c.rows, c.vocab, o.ignore, (float)o.cap, o.z_loss,
                                 o.reduction, lse.data_ptr<float>(), d.data_ptr<float>(), out.data_ptr(), c.vocab,
                                 stream_of(c.x.device()));
   }
@@ -606,7 +607,7 @@ PyObject* op_qk_norm_rope_grad(PyObject*, PyObject* const* a, Py_ssize_t na) {
 }
 
 // the arguments ignore_index, softcap, z_loss, reduction
-LossOptions loss_args(PyObject* const* a) { return {integer(a[0]), (float)number(a[1]), (float)number(a[2]), (int)integer(a[3])}; }
+LossOptions loss_args(PyObject* const* a) { return {integer(a[0]), number(a[1]), (float)number(a[2]), (int)integer(a[3])}; }
 
 // cross_entropy(logits, targets, ignore_index, softcap, z_loss, reduction) -> loss
 PyObject* op_cross_entropy(PyObject*, PyObject* const* a, Py_ssize_t na) {

@@ -44,3 +44,15 @@ def test_cross_entropy_with_large_caps(dev, dtype, rows, vocab, softcap):
     leaf = x.clone().requires_grad_(True)
     cross_entropy(leaf, t, reduction="sum", softcap=softcap).backward()
     _within(leaf.grad, want, dslack + 4 * EPS * want.abs(), "autograd")
+
+
+def test_cross_entropy_refuses_a_cap_that_is_no_float(dev):
+    """A cap that float32 rounds to zero is no missing one."""
+    from dion_amd import cross_entropy, cross_entropy_with_grad
+    from dion_amd._lib import DionAmdError
+
+    z, t = torch.randn(3, 10, device=dev), torch.zeros(3, dtype=torch.long, device=dev)
+    for cap in (1e-50, -1e-50, 1e50, math.nan):
+        for call in (cross_entropy, cross_entropy_with_grad):
+            with pytest.raises(DionAmdError, match="positive number"):
+                call(z, t, softcap=cap)
