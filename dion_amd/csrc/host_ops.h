@@ -337,7 +337,8 @@ void run_cross_entropy(const at::Tensor& logits, const at::Tensor& targets, cons
 at::Tensor run_cross_entropy_grad(const at::Tensor& logits, const at::Tensor& targets, const LossOptions& o, const at::Tensor& lse,
                                   const at::Tensor& dloss) {
   const LossCall c(logits, targets, o);
-  const at::Tensor d = dloss.to(at::kFloat).contiguous();
+  const at::Tensor d = dloss.to(at::kFloat).contiguous().resolve_neg();
+  same_device(d, logits, "cross_entropy", "the upstream gradient");
   const c10::DeviceGuard guard(c.x.device());
   const at::Tensor out = at::empty(logits.sizes(), c.x.options());
   int rc;

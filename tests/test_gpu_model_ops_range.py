@@ -56,3 +56,19 @@ def test_cross_entropy_refuses_a_cap_that_is_no_float(dev):
         for call in (cross_entropy, cross_entropy_with_grad):
             with pytest.raises(DionAmdError, match="positive number"):
                 call(z, t, softcap=cap)
+
+
+def test_negated_upstream_gradient_of_the_loss(dev):
+    """The upstream gradient may be a tensor whose memory holds the negative of its values."""
+    from dion_amd import cross_entropy
+
+    z, t = torch.randn(3, 10, device=dev), torch.tensor([1, 4, 9], device=dev)
+    for reduction, up in (("mean", torch.randn((), device=dev)), ("none", torch.randn(3, device=dev))):
+        negated = torch.complex(torch.zeros_like(up), -up).conj().imag
+        assert negated.is_neg() and torch.equal(negated, up)
+        grads = []
+        for d in (up, negated):
+            leaf = z.clone().requires_grad_(True)
+            cross_entropy(leaf, t, reduction=reduction).backward(d)
+            grads.append(leaf.grad)
+        assert torch.equal(*grads)
