@@ -72,6 +72,9 @@ at::Tensor rows_of(const at::Tensor& t) {
 }
 long long pitch(const at::Tensor& t) { return t.size(0) <= 1 ? t.size(1) : t.stride(0); }
 
+// A tensor of the caller's is about to be written over: what autograd has kept of it must not go unnoticed.
+void written(const at::Tensor& t) { t.unsafeGetTensorImpl()->bump_version(); }
+
 // Memory of the current device and stream for the length of a call: what is enqueued later on the stream may have it next.  (The
 // allocator itself, without a tensor around it: 1 us less a call.)
 at::DataPtr scratch(size_t nbytes) { return nbytes ? c10::hip::HIPCachingAllocator::get()->allocate(nbytes) : at::DataPtr(); }
@@ -124,7 +127,8 @@ at::Tensor run_embedding_grad(const at::Tensor& grad, const at::Tensor& ids, lon
   }
   const at::Tensor g = rows_of(grad.reshape({ids.numel(), dim})), t = ids.contiguous();
   const c10::DeviceGuard guard(grad.device());
-  if (!out.defined()) out = at::empty({vocab, dim}, grad.options().dtype(type));
+  if (out.defined()) written(out);
+  else out = at::empty({vocab, dim}, grad.options().dtype(type));
   const int wc = float_code(out, op, "the result");
   const size_t need = ops.embedding_grad_bytes(t.numel(), vocab, (int)dim);
   const at::DataPtr ws = scratch(need);

@@ -72,3 +72,16 @@ def test_negated_upstream_gradient_of_the_loss(dev):
             cross_entropy(leaf, t, reduction=reduction).backward(d)
             grads.append(leaf.grad)
         assert torch.equal(*grads)
+
+
+# ------------------------------------------------------------------------------------------------------------- autograd
+def test_given_table_gradient_counts_as_modified(dev):
+    from dion_amd import embedding_backward
+
+    grad, tokens = torch.randn(3, 8, device=dev), torch.tensor([1, 4, 1], device=dev)
+    for accumulate in (False, True):
+        out, leaf = torch.randn(10, 8, device=dev), torch.randn(10, 8, device=dev, requires_grad=True)
+        loss = (leaf * out).sum()
+        embedding_backward(grad, tokens, 10, out=out, accumulate=accumulate)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            loss.backward()
