@@ -575,6 +575,7 @@ PyObject* op_qk_norm_rope(PyObject*, PyObject* const* a, Py_ssize_t na) {
   return guarded(op, 9, na, [&] {
     const QkInputs in = qk_args(a, op);
     const bool track = wants_grad(op, {in.x, in.x + 1, in.gain, in.gain + 1});
+    if (wants_grad(op, {&in.cos, &in.sin})) refuse(op, "cos and sin are constants, without a gradient of their own (detach them)");
     at::Tensor out[2];
     {
       const at::NoGradGuard no_grad;

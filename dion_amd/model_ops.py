@@ -68,8 +68,8 @@ def qk_norm_rope(q: Tensor, k: Tensor, cos: Tensor, sin: Tensor, *, q_gain: Opti
 
     q: (batch, length, heads, channels), k the same with heads of its own; any strides with contiguous channels, so that both
     may be slices of one projection's output.  The results are contiguous.
-    cos, sin: float32 (positions, rotary / 2), see `rope_tables`.  The pairs (i, i + rotary / 2) are turned, the pairs
-    (2i, 2i + 1) if `interleaved`; channels from `rotary` on are only normed.
+    cos, sin: float32 (positions, rotary / 2), see `rope_tables`; constants, refused if a gradient of theirs is wanted.
+    The pairs (i, i + rotary / 2) are turned, the pairs (2i, 2i + 1) if `interleaved`; channels from `rotary` on are only normed.
     q_gain, k_gain: a factor for each channel.  positions: (length) or (batch, length), default 0, 1, 2, ...; a position outside
     the tables gives NaN."""
     return _lib.host().qk_norm_rope(q, k, cos, sin, q_gain, k_gain, positions, eps, interleaved)

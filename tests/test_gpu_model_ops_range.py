@@ -85,3 +85,21 @@ def test_given_table_gradient_counts_as_modified(dev):
         embedding_backward(grad, tokens, 10, out=out, accumulate=accumulate)
         with pytest.raises(RuntimeError, match="modified by an inplace operation"):
             loss.backward()
+
+
+def test_rotation_tables_that_want_a_gradient_are_refused(dev):
+    import dion_amd as A
+    from dion_amd._lib import DionAmdError
+
+    x = torch.randn(1, 3, 2, 8, device=dev)
+    cos, sin = A.rope_tables(3, 8, device=dev)
+    for tables in ((cos.clone().requires_grad_(True), sin), (cos, sin.clone().requires_grad_(True))):
+        with pytest.raises(DionAmdError, match="cos and sin are constants"):
+            A.qk_norm_rope(x, x, *tables)
+        with torch.no_grad():
+            q, _ = A.qk_norm_rope(x, x, *tables)
+        assert torch.equal(q, A.qk_norm_rope(x, x, cos, sin)[0])
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(sin, torch.ones_like(sin))
+        with pytest.raises(DionAmdError, match="forward mode"):
+            A.qk_norm_rope(x, x, cos, dual)
