@@ -365,6 +365,11 @@ using torch::autograd::edge_list;
 using torch::autograd::set_history;
 using torch::autograd::variable_list;
 
+// A tangent would be lost.
+void no_tangent(const at::Tensor& t, const std::string& op) {
+  if (t.defined() && t._fw_grad(0).defined()) refuse(op.c_str(), "no gradient in forward mode");
+}
+
 struct OperatorNode : torch::autograd::Node {
   // the gradients of the inputs, from those of the outputs; called with gradients off
   virtual variable_list gradients(const variable_list& grads) = 0;
@@ -377,6 +382,7 @@ struct OperatorNode : torch::autograd::Node {
   }
   variable_list apply(variable_list&& grads) override {
     const std::lock_guard<std::mutex> lock(mutex_);
+    for (const at::Tensor& g : grads) no_tangent(g, name());
     const bool twice = at::GradMode::is_enabled();   // a graph of the gradients is wanted
     variable_list out;
     {
@@ -443,9 +449,8 @@ std::shared_ptr<N> make_node() { return {new N(), deleteNode}; }   // (a long gr
 bool wants_grad(const char* op, std::initializer_list<const at::Tensor*> inputs) {
   bool wants = false;
   for (const at::Tensor* t : inputs) {
-    if (!t->defined()) continue;
-    if (t->_fw_grad(0).defined()) refuse(op, "no gradient in forward mode");
-    wants = wants || t->requires_grad();
+    no_tangent(*t, op);
+    wants = wants || (t->defined() && t->requires_grad());
   }
   return wants && at::GradMode::is_enabled();
 }
@@ -557,6 +562,7 @@ PyObject* op_embedding_grad(PyObject*, PyObject* const* a, Py_ssize_t na) {
     const at::NoGradGuard no_grad;
     const at::Tensor &grad = tensor_arg(a[0], op, "grad"), &tokens = tensor_arg(a[1], op, "tokens");
     const at::Tensor out = optional_arg(a[6], op, "out");
+    for (const at::Tensor* t : {&grad, &out}) no_tangent(*t, op);
     const at::ScalarType type = dtype_arg(a[5], out.defined() ? out.scalar_type() : grad.scalar_type(), op);
     return wrap(run_embedding_grad(grad, tokens, integer(a[2]), integer(a[3]), (float)number(a[4]), type, out, truth(a[7])));
   });
@@ -606,6 +612,7 @@ PyObject* op_qk_norm_rope_grad(PyObject*, PyObject* const* a, Py_ssize_t na) {
     const at::NoGradGuard no_grad;
     const QkInputs in = qk_args(a, op);
     const at::Tensor dy[2] = {tensor_arg(a[9], op, "dq"), tensor_arg(a[10], op, "dk")};
+    for (const at::Tensor* t : {in.x, in.x + 1, &in.cos, &in.sin, in.gain, in.gain + 1, dy, dy + 1}) no_tangent(*t, op);
     at::Tensor out[4];
     run_qk_norm_rope_grad(in, dy, out);
     return wrap_all(out);
@@ -648,6 +655,7 @@ PyObject* op_cross_entropy_with_grad(PyObject*, PyObject* const* a, Py_ssize_t n
     const at::Tensor &logits = tensor_arg(a[0], op, "logits"), &targets = tensor_arg(a[1], op, "targets");
     const LossOptions options = loss_args(a + 2);
     const bool inplace = truth(a[7]);
+    no_tangent(logits, op);
     at::Tensor out[3];
     // (the gradient is no part of the logits' graph, also where it takes their place)
     run_cross_entropy(inplace ? logits.detach() : logits, targets, options, false, inplace ? 2 : 1, (float)number(a[6]), out);

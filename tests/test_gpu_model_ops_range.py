@@ -103,3 +103,27 @@ def test_rotation_tables_that_want_a_gradient_are_refused(dev):
         dual = torch.autograd.forward_ad.make_dual(sin, torch.ones_like(sin))
         with pytest.raises(DionAmdError, match="forward mode"):
             A.qk_norm_rope(x, x, cos, dual)
+
+
+def test_tangents_are_refused_by_the_gradients(dev):
+    """What the gradients would have to do with a tangent they do not: none is dropped without a word."""
+    import dion_amd as A
+    from dion_amd._lib import DionAmdError
+
+    w, t = torch.randn(3, 8, device=dev), torch.tensor([1, 4, 1], device=dev)
+    x = torch.randn(1, 3, 2, 8, device=dev)
+    cos, sin = A.rope_tables(3, 8, device=dev)
+    gain = torch.rand(8, device=dev)
+    table, q, z = (a.clone().requires_grad_(True) for a in (torch.randn(5, 8, device=dev), x, w))
+    with torch.autograd.forward_ad.dual_level():
+        dual = lambda a: torch.autograd.forward_ad.make_dual(a.detach().clone(), torch.ones_like(a))  # noqa: E731
+        for call in (lambda: A.embedding_backward(dual(w), t, 5), lambda: A.embedding_backward(w, t, 5, out=dual(table), accumulate=True),
+                     lambda: A.qk_norm_rope_backward(dual(x), x, x, x, cos, sin), lambda: A.qk_norm_rope_backward(x, x, x, dual(x), cos, sin),
+                     lambda: A.qk_norm_rope_backward(x, x, x, x, dual(cos), sin),
+                     lambda: A.qk_norm_rope_backward(x, x, x, x, cos, sin, q_gain=dual(gain), k_gain=gain),
+                     lambda: A.cross_entropy_with_grad(dual(w), t), lambda: A.cross_entropy_with_grad(dual(w), t, inplace=True)):
+            with pytest.raises(DionAmdError, match="forward mode"):
+                call()
+        for out, leaf in ((A.embedding(table, t), table), (A.qk_norm_rope(q, x, cos, sin)[0], q), (A.cross_entropy(z, t, reduction="none"), z)):
+            with pytest.raises(RuntimeError, match="forward mode"):
+                torch.autograd.grad(out, leaf, dual(out))
