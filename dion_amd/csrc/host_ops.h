@@ -510,7 +510,7 @@ PyObject* wrap_all(const at::Tensor (&ts)[N]) {
   return out;
 }
 
-// Runs `body` with the exceptions of C++ turned into Python's.
+// Runs `body` with the exceptions of C++ turned into Python's: ATen's as its own operators do, those of Python (a hook's) as they are.
 template <typename F>
 PyObject* guarded(const char* op, Py_ssize_t want, Py_ssize_t got, F&& body) {
   if (want != got) {
@@ -522,8 +522,8 @@ PyObject* guarded(const char* op, Py_ssize_t want, Py_ssize_t got, F&& body) {
   } catch (const Failed&) {
   } catch (const Refused& e) {
     PyErr_SetString(g_error, e.what());
-  } catch (const std::exception& e) {
-    PyErr_SetString(PyExc_RuntimeError, e.what());
+  } catch (const std::exception&) {
+    torch::translate_exception_to_python(std::current_exception());
   }
   return nullptr;
 }

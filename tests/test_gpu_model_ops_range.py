@@ -127,3 +127,32 @@ def test_tangents_are_refused_by_the_gradients(dev):
         for out, leaf in ((A.embedding(table, t), table), (A.qk_norm_rope(q, x, cos, sin)[0], q), (A.cross_entropy(z, t, reduction="none"), z)):
             with pytest.raises(RuntimeError, match="forward mode"):
                 torch.autograd.grad(out, leaf, dual(out))
+
+
+def test_exceptions_keep_their_type(dev):
+    """No memory is torch.OutOfMemoryError, as of any operator; an exception of a hook on saved tensors is that exception."""
+    import dion_amd as A
+
+    w, t = torch.randn(10, 8, device=dev, requires_grad=True), torch.tensor([1, 4, 1], device=dev)
+    x = torch.randn(1, 3, 2, 8, device=dev, requires_grad=True)
+    z = torch.randn(3, 10, device=dev, requires_grad=True)
+    cos, sin = A.rope_tables(3, 8, device=dev)
+
+    def pack(tensor):
+        raise KeyError("packed")
+
+    with torch.autograd.graph.saved_tensors_hooks(pack, lambda tensor: tensor):
+        for call in (lambda: A.embedding(w, t), lambda: A.qk_norm_rope(x, x, cos, sin), lambda: A.cross_entropy(z, t)):
+            with pytest.raises(KeyError, match="packed"):
+                call()
+    torch.cuda.empty_cache()
+    total = torch.cuda.get_device_properties(dev).total_memory
+    # the allocator's own limit, a little above what is in use: nothing is asked of the device
+    torch.cuda.set_per_process_memory_fraction((torch.cuda.memory_reserved(dev) + (64 << 20)) / total, dev)
+    try:
+        with pytest.raises(torch.OutOfMemoryError):
+            A.embedding(w.detach(), t[:1].expand(1 << 24))
+        with pytest.raises(torch.OutOfMemoryError):
+            A.embedding_backward(torch.randn(3, 8, device=dev), t, 1 << 24)
+    finally:
+        torch.cuda.set_per_process_memory_fraction(1.0, dev)
