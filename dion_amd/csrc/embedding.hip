@@ -571,7 +571,7 @@ __global__ __launch_bounds__(256) void embedding_join_kernel(RowArgs a, int slic
   const int lane = threadIdx.x % DA_WAVE, wave = threadIdx.x / DA_WAVE;
   const int column = blockIdx.x % slices * DA_WAVE + lane;
   int skip;
-  const int c = da_column<COLS>(column, a.dim, skip);
+  const int c = da_column<COLS>(column < a.lanes ? column : a.lanes - 1, a.dim, skip);
   // partial sum 0 is the back of this piece, i > 0 the front of piece + i
   const int n = (range.x + range.y - 1) / a.piece - piece + 1, quarter = (n + 3) / 4;
   const int begin = wave * quarter, end = begin + quarter < n ? begin + quarter : n;
@@ -619,7 +619,7 @@ GradPlan plan_grad(long long count, long long vocab, int dim, int g_dtype) {
   GradPlan p{};
   const int wide = g_dtype == DA_BF16 ? 8 : 4;   // 16 bytes of the gradient
   p.cols = dim >= wide ? wide : 1;
-  p.lanes = (dim + p.cols - 1) / p.cols;
+  p.lanes = da_lanes(dim, p.cols);
   p.log2_bins = 8;
   while ((vocab >> p.log2_bins) + 1 > IDX_ROWS) ++p.log2_bins;
   const long long bins = 1ll << p.log2_bins;
@@ -725,7 +725,7 @@ int dion_amd_embedding(const void* W, int w_dtype, long long ldw, long long voca
   hipStream_t s = static_cast<hipStream_t>(stream);
   const DaIndex idx{tokens, index_bits == 64};
   DaProfScope prof(DA_PROF_EMBEDDING, (double)count * dim * (da_esize(w_dtype) + da_esize(out_dtype)), s);
-  const int cols = dim >= 8 ? 8 : 1, lanes = (dim + cols - 1) / cols;
+  const int cols = dim >= 8 ? 8 : 1, lanes = da_lanes(dim, cols);
   if (count * lanes >= (1ll << 32) - 256 * UNITS) return DA_ERR_LIMIT;
   const dim3 grid((unsigned)((count * lanes + 256 * UNITS - 1) / (256 * UNITS)));
   const DaDivisor by_lanes = da_divisor((unsigned)lanes);

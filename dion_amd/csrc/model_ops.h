@@ -63,6 +63,8 @@ __device__ __forceinline__ float da_group_max(float v, int log2_group = 6) {
 }
 
 __host__ inline size_t da_esize(int dtype) { return dtype == DA_BF16 ? 2 : 4; }
+// Lanes of a row of dim elements, cols to a lane (dim up to 2^31 - 1).
+__host__ inline int da_lanes(int dim, int cols) { return dim / cols + (dim % cols != 0); }
 __host__ inline bool da_float_dtype(int dtype) { return dtype == DA_BF16 || dtype == DA_F32; }
 __host__ inline bool da_aligned(const void* p, size_t bytes) { return (reinterpret_cast<uintptr_t>(p) % bytes) == 0; }
 

@@ -156,3 +156,15 @@ def test_exceptions_keep_their_type(dev):
             A.embedding_backward(torch.randn(3, 8, device=dev), t, 1 << 24)
     finally:
         torch.cuda.set_per_process_memory_fraction(1.0, dev)
+
+
+# ------------------------------------------------------------------------------------------------------------ embedding
+def test_embedding_of_the_widest_rows(dev):
+    """Rows whose width rounded up to whole lanes is past 2^31."""
+    from dion_amd import embedding, embedding_backward
+
+    dim = 2 ** 31 - 1
+    row = torch.randn(1, dim, device=dev, dtype=BF)
+    token = torch.zeros(1, dtype=torch.long, device=dev)
+    assert torch.equal(embedding(row, token), row)
+    assert torch.equal(embedding_backward(row, token, 1), row)
