@@ -271,19 +271,24 @@ __global__ __launch_bounds__(256) void qk_heads_grad_kernel(QkArgs a) {
     float u[PAIRS], v[PAIRS], du[PAIRS], dv[PAIRS];
     it.x.template pairs<INTER>(u, v);
     it.d.template pairs<INTER>(du, dv);
-    float own_u[PAIRS], own_v[PAIRS];
+    if (at.table >= 0) turn<PAIRS, true>(du, dv, c, s);
+    float own_u[PAIRS], own_v[PAIRS], wu[PAIRS], wv[PAIRS];
 #pragma unroll
     for (int i = 0; i < PAIRS; ++i) {
       own_u[i] = u[i];
       own_v[i] = v[i];
+      wu[i] = du[i] * gu[i];
+      wv[i] = dv[i] * gv[i];
     }
-    if (RAGGED) leave<PAIRS, INTER>(at, own_u, own_v);
-    if (at.table >= 0) turn<PAIRS, true>(du, dv, c, s);
+    if (RAGGED) {   // both factors: what another lane counts may be infinite
+      leave<PAIRS, INTER>(at, own_u, own_v);
+      leave<PAIRS, INTER>(at, wu, wv);
+    }
     float square = 0.f, dot = 0.f;
 #pragma unroll
     for (int i = 0; i < PAIRS; ++i) {
       square = fmaf(own_u[i], own_u[i], fmaf(own_v[i], own_v[i], square));
-      dot = fmaf(du[i] * gu[i], own_u[i], fmaf(dv[i] * gv[i], own_v[i], dot));
+      dot = fmaf(wu[i], own_u[i], fmaf(wv[i], own_v[i], dot));
     }
     square = da_group_sum(square, a.log2_group);
     dot = da_group_sum(dot, a.log2_group);

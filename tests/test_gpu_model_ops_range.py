@@ -168,3 +168,25 @@ def test_embedding_of_the_widest_rows(dev):
     token = torch.zeros(1, dtype=torch.long, device=dev)
     assert torch.equal(embedding(row, token), row)
     assert torch.equal(embedding_backward(row, token, 1), row)
+
+
+# ---------------------------------------------------------------------------------------------------------- q / k norms
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("dim, rotary, interleaved", [(80, 40, False), (90, 44, True), (72, 24, False), (96, 96, True), (128, 128, False)])
+def test_qk_norm_rope_gradient_of_infinite_upstream_values(dev, dtype, dim, rotary, interleaved):
+    """Infinities and NaN stand where the definition has them, whichever lanes hold the channel."""
+    from dion_amd import qk_norm_rope_backward, rope_tables
+    from oracle import model_ops as O
+
+    g = _gen(dim)
+    q, k = torch.randn(1, dim + 1, 2, dim, generator=g).to(dtype), torch.randn(1, dim + 1, 1, dim, generator=g).to(dtype)
+    cos, sin = rope_tables(dim + 1, rotary)
+    gain = torch.rand(dim, generator=g) + 0.5
+    dy = torch.randn(1, dim + 1, 2, dim, generator=g).to(dtype)
+    for channel in range(dim):      # a token each, behind the first, whose angle is zero
+        dy[0, channel + 1, 0, channel] = math.inf
+    (want, _), _ = O.norm_rope_grad(dy, q, cos, sin, gain, interleaved=interleaved)
+    got = qk_norm_rope_backward(*(a.to(dev) for a in (dy, k, q, k, cos, sin)), q_gain=gain.to(dev), interleaved=interleaved)[0].cpu().double()
+    assert torch.equal(got.isnan(), want.isnan()) and want[0, 1:, 0].isinf().any(-1).sum() > dim // 4
+    assert torch.equal(got == math.inf, want == math.inf) and torch.equal(got == -math.inf, want == -math.inf)
+    assert got[0, :, 1].isfinite().all()
