@@ -621,7 +621,7 @@ GradPlan plan_grad(long long count, long long vocab, int dim, int g_dtype) {
   p.cols = dim >= wide ? wide : 1;
   p.lanes = da_lanes(dim, p.cols);
   p.log2_bins = 8;
-  while ((vocab >> p.log2_bins) + 1 > IDX_ROWS) ++p.log2_bins;
+  while (vocab > (long long)IDX_ROWS << p.log2_bins) ++p.log2_bins;
   const long long bins = 1ll << p.log2_bins;
   p.rows = (int)((vocab + bins - 1) / bins);
   p.range = 0;

@@ -7,7 +7,7 @@ import math
 import pytest
 import torch
 
-from test_gpu_model_ops import BF, EPS, F32, _gen, _loss_problem, _qk_problem, _within
+from test_gpu_model_ops import BF, EPS, F32, _check_table_gradient, _gen, _loss_problem, _qk_problem, _within
 
 pytestmark = pytest.mark.gpu
 
@@ -190,3 +190,13 @@ def test_qk_norm_rope_gradient_of_infinite_upstream_values(dev, dtype, dim, rota
     assert torch.equal(got.isnan(), want.isnan()) and want[0, 1:, 0].isinf().any(-1).sum() > dim // 4
     assert torch.equal(got == math.inf, want == math.inf) and torch.equal(got == -math.inf, want == -math.inf)
     assert got[0, :, 1].isfinite().all()
+
+
+@pytest.mark.parametrize("vocab", [262143, 262144, 262145])
+@pytest.mark.parametrize("count", [100, 3000, 30000])
+def test_embedding_backward_of_full_bins(dev, count, vocab):
+    """Bins of exactly as many ids as the index has threads, and one more id."""
+    g = _gen(count)
+    tokens = torch.randint(0, vocab, (count,), generator=g)
+    tokens[:6] = torch.tensor([vocab - 1, 0, vocab - 1, vocab - 256, 255, vocab - 1])
+    _check_table_gradient(dev, torch.randn(count, 5, generator=g), tokens, vocab, F32, padding_idx=255)
