@@ -200,3 +200,74 @@ def test_embedding_backward_of_full_bins(dev, count, vocab):
     tokens = torch.randint(0, vocab, (count,), generator=g)
     tokens[:6] = torch.tensor([vocab - 1, 0, vocab - 1, vocab - 256, 255, vocab - 1])
     _check_table_gradient(dev, torch.randn(count, 5, generator=g), tokens, vocab, F32, padding_idx=255)
+
+
+def _grad_on_gpu(grad, tokens, vocab):
+    """(gradient, sum of absolute terms, number of terms of a row) in float64, on the GPU"""
+    g = grad.double()
+    total = torch.zeros(vocab, g.size(1), dtype=torch.float64, device=g.device)
+    magnitude, count = torch.zeros_like(total), torch.bincount(tokens, minlength=vocab)
+    return total.index_add_(0, tokens, g), magnitude.index_add_(0, tokens, g.abs()), count
+
+
+def _check_on_gpu(grad, tokens, vocab, dtype):
+    from dion_amd import embedding_backward
+
+    got = embedding_backward(grad, tokens, vocab, dtype=dtype)
+    want, magnitude, count = _grad_on_gpu(grad, tokens, vocab)
+    off = (got.double() - want).abs() - (2.0 ** (-8 if dtype == BF else -24) * want.abs() + 1.01 * (count[:, None] + 2) * EPS * magnitude + 1e-38)
+    assert off.max() <= 0, f"{off.max().item():.3e} beyond the bound"
+    assert torch.equal(got, embedding_backward(grad, tokens, vocab, dtype=dtype)), "not the same bits twice"
+
+
+# Entries of a piece are 32 from 4.2 million pairs of token and lane on, 16 from 2.1 million: (tokens, columns) that reach either in
+# bf16 (8 columns a lane) and fp32 (4), by the index of few tokens and by that of sorted parts.
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("count, dim", [(5001, 2048), (9001, 2049), (20000, 2048), (70001, 512)])
+def test_embedding_backward_of_long_pieces(dev, count, dim, dtype):
+    g = torch.Generator(dev).manual_seed(count)
+    vocab = 5000
+    u = torch.rand(count, generator=g, device=dev, dtype=torch.float64)
+    i = torch.arange(count, device=dev)
+    zipf = (2.7 * ((vocab + 2.7) / 2.7) ** u - 2.7).long().clamp(0, vocab - 1)
+    grad = torch.randn(count, dim, generator=g, device=dev, dtype=dtype)
+    for tokens in (zipf, i // 97 % vocab, torch.full_like(i, 4321), torch.where(i % 5 == 3, 4321, zipf), torch.where(u < 0.3, 0, zipf)):
+        _check_on_gpu(grad, tokens, vocab, dtype)
+
+
+@pytest.mark.parametrize("dtype, dim", [(BF, 72), (F32, 72), (BF, 16392), (F32, 8196), (BF, 32768), (F32, 16384)])
+def test_embedding_backward_around_the_borders_of_pieces(dev, dtype, dim):
+    """One id between two others of its bin, its run beginning and ending at every distance from the borders of pieces of 8, 16 and 32
+    entries (by the widths), in calls too long for one launch."""
+    g = torch.Generator(dev).manual_seed(dim)
+    grad = torch.randn(1100, dim, generator=g, device=dev, dtype=dtype)
+    for lead in (0, 1, 7, 8, 9, 15, 16, 17, 31, 32, 33, 63, 64):
+        for run in (1050 - lead, 1023, 33):
+            tokens = torch.cat([torch.full((n,), id, device=dev) for n, id in ((lead, 2), (run, 258), (1100 - lead - run, 514))])
+            _check_on_gpu(grad, tokens[torch.randperm(1100, generator=g, device=dev)], 600, dtype)
+
+
+@pytest.mark.parametrize("dtype, gain_dtype", [(BF, F32), (F32, BF), (BF, BF), (F32, F32)])
+@pytest.mark.parametrize("case", [(7, 1021, 6, 2, 90, 44, True, True, True), (2, 2051, 32, 8, 128, 128, False, True, True),
+                                  (2, 1500, 3, 1, 22, 6, False, True, True), (5, 901, 12, 12, 64, 48, False, True, True)])
+def test_qk_norm_rope_gradient_of_many_heads(dev, case, dtype, gain_dtype):
+    """More heads than the workgroups of a gradient with gains have lane groups, so that each takes several, and a ragged rest; the
+    oracle runs on the GPU, in float64."""
+    from dion_amd import qk_norm_rope_backward
+    from oracle import model_ops as O
+
+    q, k, cos, sin, options, dy = _qk_problem(dev, case, dtype, gain_dtype)
+    grads = qk_norm_rope_backward(*dy, q, k, cos, sin, **options)
+    d = q.size(-1)
+    for w, (x, name) in enumerate(((q, "q"), (k, "k"))):
+        (dx, mx), (dgain, mg) = O.norm_rope_grad(dy[w], x, cos, sin, options[name + "_gain"], options["positions"], 1e-6, options["interleaved"])
+        u = 2.0 ** (-8 if dtype == BF else -24)
+        off = (grads[w].double() - dx).abs() - (u * dx.abs() + 1.01 * (2 * d + 24) * EPS * mx + 1e-38)
+        assert off.max() <= 0, f"d{name}: {off.max().item():.3e} beyond the bound"
+        # a term of the gain's gradient (d + 24), and the additions that it passes through: at most 32 heads of a lane group, 8 between the
+        # lanes and wavefronts, 32 where the workgroups are joined
+        u = 2.0 ** (-8 if gain_dtype == BF else -24)
+        off = (grads[2 + w].double() - dgain).abs() - (u * dgain.abs() + 1.01 * (d + 24 + 72) * EPS * mg + 1e-38)
+        assert off.max() <= 0, f"gain of {name}: {off.max().item():.3e} beyond the bound"
+    for a, b in zip(grads, qk_norm_rope_backward(*dy, q, k, cos, sin, **options)):
+        assert torch.equal(a, b), "not the same bits twice"
