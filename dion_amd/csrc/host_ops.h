@@ -122,6 +122,10 @@ at::Tensor run_embedding_grad(const at::Tensor& grad, const at::Tensor& ids, lon
     if (out.dim() != 2 || out.size(0) != vocab || out.size(1) != dim || (dim > 1 && out.stride(1) != 1) || (vocab > 1 && out.stride(0) < dim))
       refuse(op, "out must be (num_embeddings, columns) with contiguous rows");
     if (out.scalar_type() != type) refuse(op, "dtype is not that of out");
+    for (const at::Tensor* t : {&grad, &ids}) {   // (tables with gaps may lie between the rows of others)
+      const at::MemOverlapStatus over = at::get_overlap_status(out, *t);
+      if (over == at::MemOverlapStatus::Full || over == at::MemOverlapStatus::Partial) refuse(op, "out and an input overlap");
+    }
   } else if (accumulate) {
     refuse(op, "accumulate needs out");
   }

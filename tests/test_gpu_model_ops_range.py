@@ -271,3 +271,20 @@ def test_qk_norm_rope_gradient_of_many_heads(dev, case, dtype, gain_dtype):
         assert off.max() <= 0, f"gain of {name}: {off.max().item():.3e} beyond the bound"
     for a, b in zip(grads, qk_norm_rope_backward(*dy, q, k, cos, sin, **options)):
         assert torch.equal(a, b), "not the same bits twice"
+
+
+def test_table_gradient_over_its_own_input_is_refused(dev):
+    """A table that lies over the gradient it is made from; one beside it in the same rows is taken."""
+    from dion_amd import embedding_backward
+    from dion_amd._lib import DionAmdError
+
+    both = torch.randn(600, 24, device=dev)
+    tokens = torch.randint(0, 600, (600,), generator=_gen(1)).to(dev)
+    grad = both[:, :8].contiguous()
+    want = embedding_backward(grad, tokens, 600)
+    for out in (grad, grad.view(-1)[:4800].view(600, 8)):
+        with pytest.raises(DionAmdError, match="overlap"):
+            embedding_backward(grad, tokens, 600, out=out)
+    with pytest.raises(DionAmdError, match="overlap"):
+        embedding_backward(grad[:500], tokens[:500], 500, out=grad[100:])
+    assert torch.equal(embedding_backward(both[:, :8], tokens, 600, out=both[:, 8:16]), want) and torch.equal(both[:, 8:16], want)
