@@ -186,12 +186,12 @@ __device__ __forceinline__ void gradient(const CeArgs& a, float (&x)[N], int fir
 
 // ---- a row in the registers of one workgroup: loss and gradient from one read
 //
-// A thread holds up to VECS vectors of 16 bytes of the row (24 at the most: 114 registers), and one element of its end where that is no whole vector.  The maximum
-// and the sum are each thread's own until the one exchange between the wavefronts.
+// A thread holds up to VECS vectors of 16 bytes of the row (24 at the most: 113 registers, 119 with a wide cap), and one element of its
+// end where that is no whole vector.  The maximum and the sum are each thread's own until the one exchange between the wavefronts.
 //
 // 16384 rows of 50304 bf16 classes, a tenth of them ignored: 550-580 us for 2.92 GiB (5.4-5.7 TB/s; read twice, 2000 with the plain
-// two passes).  19 cycles a lane and element without a cap, 36 with one in bf16, where the arithmetic bounds it (4.4 TB/s).  Two
-// workgroups a compute unit take turns at memory and arithmetic; rows of more than 8192 vectors leave room for one (4.0 TB/s with 18992
+// two passes).  19 cycles a lane and element without a cap; a small one in bf16 takes 36 and a wide one half as many again, where the
+// arithmetic bounds it (8192 rows of 50304 classes 390 and 560 us: 4.2 and 3.0 TB/s).  Two workgroups a compute unit take turns at memory and arithmetic; rows of more than 8192 vectors leave room for one (4.0 TB/s with 18992
 // vectors: 2048 rows of 151936 bf16 classes in 312 us, 383 if they are read twice).
 template <typename T, Cap CAP, int THREADS, int VECS>
 __global__ __launch_bounds__(THREADS) void ce_row_kernel(CeArgs a) {
@@ -281,8 +281,8 @@ __global__ __launch_bounds__(THREADS) void ce_row_kernel(CeArgs a) {
 // ---- rows in slices: the loss alone, rows too long for the registers, and few rows that have to share the chip
 //
 // Statistics: a thread requests its next four vectors before it works on four.  2047 rows of 50257 bf16 classes with a cap, 206 MB in
-// 46-50 us (with 256 threads in place of 1024, and without the request ahead, 43-57); 8192 of 50304 without one 171 us (4.8 TB/s; 256
-// threads 186).  16 rows of 128000 fp32 classes in 7 slices: 4.6 us and 2.2 for the join, from one workgroup a row 73.
+// 46-50 us (with 256 threads in place of 1024, and without the request ahead, 43-57); 8192 of 50304 without one 134 us (6.1
+// TB/s).  16 rows of 128000 fp32 classes in 7 slices: 4.6 us and 2.2 for the join, from one workgroup a row 73.
 constexpr int SLICE_THREADS = 1024, SLICE_VECS = 4;
 
 // Maximum and sum of one slice of a row; of a row in one slice also its loss.
@@ -499,7 +499,8 @@ void cut(Form& f, long long vocab, int n, int slices) {
 // since a row in one slice needs no launch to join it (100 rows of 50304 bf16 classes 12.5 us, 14.7 with 2048 and 15.9 with two
 // workgroups a compute unit; 400 rows 22.6, 22.6 and 26.3; with the gradient 64 rows 17.5, 16.8 and 17.4).
 // Without a gradient, rows of up to 2048 vectors go to the workgroups of 256 threads that hold them: 20000 rows of 10000 bf16 classes
-// 117 us, in workgroups of 1024 168; of 16384 classes 160 and 187, but of 32000 143 and 123 (all with the sum behind).  With one, rows
+// 73 us (5.5 TB/s), in workgroups of 1024 147; of 16384 classes 115 and 158; of 32000, held by 1024, 213 and 217, but 8192 of 50304 138
+// and 134 (all with the sum behind).  With one, rows
 // are in slices if they are a quarter of the compute units or fewer: 64 rows of 50304 bf16 classes 17 us either way, 100 18.4 in
 // registers and 21 in slices.
 Form plan_form(long long rows, long long vocab, int dtype, bool grad) {

@@ -3,7 +3,7 @@
 //   out[t] = r(scale * W[tok_t])                       dW[v] = r(scale * sum of g[t] over the t with tok_t = v  (+ dW[v]))
 //
 // Both are bound by HBM: the lookup reads one row and writes one row a token, the gradient reads one row a token and writes every
-// row of the table once.  Sums are formed in fp32 in an order that depends on the tokens alone: the same bits every time.
+// row of the table once.  Sums are formed in fp32 in an order that depends on the tokens alone, on all of them: the same bits every time.
 #include "../../include/dion_amd.h"
 #include "model_ops.h"
 #include "prof.h"
@@ -58,6 +58,11 @@ __global__ __launch_bounds__(256) void embedding_kernel(const W* w, long long ld
 // tokens a launch before has sorted each part of 1024 tokens or more by bin; the workgroup gathers its run of every part, and the places of
 // the runs in their parts add up to the place where it begins.  Sorting the positions of a bin by id is then a counting sort in LDS,
 // stable because each wavefront takes a contiguous run of tokens and ranks its lanes in order.
+//
+// A frequent id keeps the one workgroup of its bin busy while the others are done: the gradient of 65536 tokens of 768 bf16 columns takes
+// 51 us, 82 if a fifth of them are one id, 198 if all are.  Tables of more ids than 256 bins hold (262144) have more bins and no sorted
+// parts, so that the work is bins times tokens: 131072 tokens of 64 columns 49 us with 262144 ids and 135 with 262145, 2^20 tokens of 16
+// columns and as many ids 1.1 ms.
 constexpr int IDX_THREADS = 1024, IDX_WAVES = IDX_THREADS / DA_WAVE;
 constexpr int IDX_ROWS = 1024;   // ids of a bin at most: one per thread in the scan
 constexpr int IDX_AHEAD = 4;     // rounds of 64 tokens requested before the first is looked at

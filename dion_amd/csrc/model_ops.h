@@ -28,7 +28,8 @@ __device__ __forceinline__ void da_indices(const DaIndex& x, const long long (&a
   }
 }
 
-// Division of any 32-bit number by one known on the host, in three instructions or four in place of some 25.
+// Division of any 32-bit number by one known on the host, in three instructions or four in place of some 25: a multiplication and a shift
+// (Granlund and Montgomery, Division by invariant integers using multiplication, 1994).
 struct DaDivisor {
   unsigned mul, shift, by;
   __device__ __forceinline__ unsigned quotient(unsigned n) const {

@@ -7,7 +7,8 @@ pass over its data in hand-written kernels, with its gradient:
   * `qk_norm_rope` / `qk_norm_rope_backward`, tables by `rope_tables`
   * `cross_entropy` / `cross_entropy_with_grad`
 
-`embedding`, `qk_norm_rope` and `cross_entropy` take part in autograd, with nodes of the native module (first gradients only).
+`embedding`, `qk_norm_rope` and `cross_entropy` take part in autograd, with nodes of the native module (first gradients only, none in
+forward mode).
 Tensors are bfloat16 or float32 on the GPU (there is no CPU or PyTorch fallback); token ids, targets and positions int64 or
 int32.  All work goes to the current stream, nothing waits for the GPU, and the results are the same bits every time.
 """
@@ -44,8 +45,9 @@ def embedding_backward(grad: Tensor, tokens: Tensor, num_embeddings: int, *, sca
                        accumulate: bool = False) -> Tensor:
     """The dense gradient of the table: row v is `scale` times the sum of `grad` over the places where `tokens` is v.
 
-    Sums are fp32 in the order of the tokens, rounded once to `dtype` (default: that of `grad`).  out: the tensor to write;
-    with accumulate=True the gradient is added to what is in it, and rows that no token names are not touched."""
+    Sums are fp32, rounded once to `dtype` (default: that of `grad`); all tokens together determine their order, so that the last bits
+    of a row may change with tokens of other rows.  out: the tensor to write, not over an input; with accumulate=True the gradient is
+    added to what is in it, and rows that no token names are not touched."""
     return _lib.host().embedding_grad(grad, tokens, num_embeddings, _padding(padding_idx, num_embeddings), scale, dtype, out,
                                       accumulate)
 
@@ -69,7 +71,8 @@ def qk_norm_rope(q: Tensor, k: Tensor, cos: Tensor, sin: Tensor, *, q_gain: Opti
     q: (batch, length, heads, channels), k the same with heads of its own; any strides with contiguous channels, so that both
     may be slices of one projection's output.  The results are contiguous.
     cos, sin: float32 (positions, rotary / 2), see `rope_tables`; constants, refused if a gradient of theirs is wanted.
-    The pairs (i, i + rotary / 2) are turned, the pairs (2i, 2i + 1) if `interleaved`; channels from `rotary` on are only normed.
+    The pairs (i, i + rotary / 2) are turned, (u, v) -> (u cos - v sin, v cos + u sin), the pairs (2i, 2i + 1) if `interleaved`;
+    channels from `rotary` on are only normed.  A model that turns the other way passes `-sin`.
     q_gain, k_gain: a factor for each channel.  positions: (length) or (batch, length), default 0, 1, 2, ...; a position outside
     the tables gives NaN."""
     return _lib.host().qk_norm_rope(q, k, cos, sin, q_gain, k_gain, positions, eps, interleaved)
@@ -94,7 +97,7 @@ def cross_entropy(logits: Tensor, targets: Tensor, *, ignore_index: int = -100, 
     """Cross entropy over the last dimension, in float32.
 
     logits: the shape of `targets` and the classes; rows at any pitch, so that padded logits go as `logits[..., :vocab]`.
-    softcap: logits are taken as `softcap * tanh(logits / softcap)` (0: as they are).  z_loss: adds `z_loss * lse ** 2`, lse the
+    softcap: logits are taken as `softcap * tanh(logits / softcap)` (0: as they are; else 1e-30 to 1e30).  z_loss: adds `z_loss * lse ** 2`, lse the
     logarithm of the sum of exponentials.  Targets equal to `ignore_index` have no loss and no gradient, and "mean" is over the
     others (NaN if there are none); any other target outside the classes gives NaN."""
     return _lib.host().cross_entropy(logits, targets, ignore_index, softcap, z_loss, _reduction(reduction))

@@ -372,13 +372,14 @@ int dion_amd_dion_step_sketch(void* const* X, const void* const* G, void* const*
  * ------------------------------------------------------------------------------------- */
 
 /* out[t] = scale * W[tokens[t]], rounded once to out_dtype.  W: vocab x dim, row pitch ldw; out: count x dim, pitch ldo.
- * A token outside 0 ... vocab - 1 gives a row of NaN.  count and vocab at most 2^25. */
+ * A token outside 0 ... vocab - 1 gives a row of NaN.  count and vocab at most 2^25, count * ceil(dim / 8) (dim < 8: count * dim)
+ * below 2^32 - 512. */
 int dion_amd_embedding(const void* W, int w_dtype, long long ldw, long long vocab, int dim, const void* tokens, int index_bits,
                        long long count, void* out, int out_dtype, long long ldo, float scale, void* stream);
 
 /* Its gradient, dense: dW[v] = scale * sum of G[t] over the t with tokens[t] = v, for every v (accumulate: added to the
- * dW that is there).  Sums in fp32, in an order fixed by the tokens; rounded once to w_dtype.  Tokens equal to `padding`
- * (-1: none) and tokens outside the table contribute nothing. */
+ * dW that is there).  Sums in fp32, in an order that all the tokens together fix; rounded once to w_dtype.  Tokens equal to
+ * `padding` (-1: none) and tokens outside the table contribute nothing.  dW overlaps no input.  count and vocab at most 2^25. */
 size_t dion_amd_embedding_grad_workspace_bytes(long long count, long long vocab, int dim);
 int dion_amd_embedding_grad(const void* G, int g_dtype, long long ldg, const void* tokens, int index_bits, long long count,
                             void* dW, int w_dtype, long long ldw, long long vocab, int dim, long long padding, float scale,
@@ -416,7 +417,9 @@ int dion_amd_qk_norm_rope_grad(const dion_amd_heads* q, const dion_amd_heads* k,
                                float eps, void* workspace, size_t workspace_bytes, void* stream);
 
 /* Cross entropy of `rows` rows of logits (pitch ld) against targets:
- *   z = softcap * tanh(x / softcap) (softcap 0: z = x; else between 1e-30 and 1e30);  lse = log sum exp z;  l = lse - z[target] + z_loss * lse^2
+ *   z = softcap * tanh(x / softcap) (softcap 0: z = x; else 1e-30 to 1e30);  lse = log sum exp z;  l = lse - z[target] + z_loss * lse^2
+ * Errors are those of fp32; of bf16 logits with caps up to 40 z is off by up to 2^-22 of the cap.  rows below 2^22, vocab at most
+ * 2^31 - 65537.
  * Rows whose target is ignore_index have the loss 0 and are not read; any other target outside the vocabulary: NaN.
  * reduction NONE: loss receives one l a row; SUM, MEAN (over the rows that are not ignored; none: NaN): one value.
  * lse (may be NULL): one a row, and behind them the number of rows that count, for dion_amd_cross_entropy_grad: rows + 1
